@@ -1,0 +1,46 @@
+"""CPU test of the GPU code's text: instruction families that no device source of the tree may hold, in any form (inline
+assembly, builtins, assembly files) and wherever it lies -- a stand-alone probe that nothing builds counts like the library.
+
+Data is written through vector stores only.  The scalar data cache is not coherent with them, so a write through it (a scalar
+store, a scalar atomic, a write-back or discard of that cache) can lose or overtake the vector stores beside it."""
+import os
+import re
+
+import pytest
+
+REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+SOURCE = re.compile(r"\.(hip|cu|cpp|cc|c|hpp|h|cuh|s|S|ll|py|sh|txt|cmake|mk)$|^Makefile$")
+FOLDERS = ("timemachine_amd", "include", "oracle", "scripts", "tests", "bench.py", "__graft_entry__.py")
+SCALAR_CACHE_WRITE = re.compile(r"(?:\b|_)s_(?:(?:scratch_|buffer_)?(?:store|atomic)_|dcache_(?:wb|discard))", re.IGNORECASE)
+
+
+def device_sources():
+    for top in FOLDERS:
+        path = os.path.join(REPO, top)
+        if os.path.isfile(path):
+            yield path
+        for folder, _, files in os.walk(path):
+            for f in files:
+                if SOURCE.search(f):
+                    yield os.path.join(folder, f)
+
+
+def hits(pattern, path):
+    with open(path, errors="replace") as fh:
+        return [f"{os.path.relpath(path, REPO)}:{n}: {line.strip()}" for n, line in enumerate(fh, 1) if pattern.search(line)]
+
+
+@pytest.mark.parametrize("op", ["store_dword", "atomic_add", "buffer_store_dwordx2", "scratch_store_dword", "buffer_atomic_or", "dcache_wb", "dcache_discard_x2"])
+def test_the_scalar_cache_pattern_finds_every_kind_of_write(op):
+    assert SCALAR_CACHE_WRITE.search(f'asm volatile("s_{op} %0, %1, 0x0")')
+    assert SCALAR_CACHE_WRITE.search(f"__builtin_amdgcn_s_{op}();")
+
+
+@pytest.mark.parametrize("op", ["s_load_dword", "s_buffer_load_dwordx4", "s_waitcnt lgkmcnt(0)", "ds_add_u64", "global_store_dword", "global_atomic_add_x2", "buffer_store_dword", "is_store_", "s_dcache_inv"])
+def test_the_scalar_cache_pattern_leaves_loads_and_vector_stores(op):
+    assert not SCALAR_CACHE_WRITE.search(f'asm volatile("{op} %0, %1")')
+
+
+def test_no_source_writes_through_the_scalar_data_cache():
+    found = [h for path in device_sources() for h in hits(SCALAR_CACHE_WRITE, path)]
+    assert not found, "\n".join(found)
