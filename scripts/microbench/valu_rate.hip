@@ -1,34 +1,29 @@
-// Issue cost of packed f32 VALU instructions on gfx950: cycles per wave-instruction of v_fma_f32, v_pk_fma_f32, v_pk_mul_f32,
-// v_pk_add_f32 and v_fma_f64 with 1, 2 and 4 waves per SIMD (8 independent accumulators per lane, s_memtime around 4096
-// instructions; every wave reports its own start and end).   hipcc --offload-arch=gfx950 -O3 pk_f32_rate.hip -o pk_f32_rate
+// Issue cost of plain VALU instructions on gfx950: cycles per wave-instruction of v_fma_f32, v_mul_f32 and v_fma_f64 with 1, 2
+// and 4 waves per SIMD (8 independent accumulators per lane, s_memtime around 4096 instructions; every wave reports its own
+// start and end).   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops valu_rate.hip -o valu_rate
 #include <hip/hip_runtime.h>
 #include <cstdio>
-typedef float v2f __attribute__((ext_vector_type(2)));
 template <int KIND> __global__ void k(long long *out, float seed) {
-    v2f a[8];
+    float a[8];
     double d[8];
     for (int i = 0; i < 8; i++) {
-        a[i].x = seed + i + threadIdx.x;
-        a[i].y = seed - i;
+        a[i] = seed + i + threadIdx.x;
         d[i] = seed * i + threadIdx.x;
     }
-    const v2f m = {1.0001f, 0.9999f}, c = {1e-7f, -1e-7f};
+    const float m = 1.0001f, c = 1e-7f;
     const long long t0 = clock64();
 #pragma unroll 1
     for (int it = 0; it < 512; it++) {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            if (KIND == 0) asm volatile("v_fma_f32 %0, %0, %1, %2" : "+v"(a[i].x) : "v"(m.x), "v"(c.x));
-            if (KIND == 1) asm volatile("v_pk_fma_f32 %0, %0, %1, %2" : "+v"(a[i]) : "v"(m), "v"(c));
-            if (KIND == 2) asm volatile("v_pk_mul_f32 %0, %0, %1" : "+v"(a[i]) : "v"(m));
-            if (KIND == 3) asm volatile("v_pk_add_f32 %0, %0, %1" : "+v"(a[i]) : "v"(c));
-            if (KIND == 4) asm volatile("v_fma_f64 %0, %0, %1, %2" : "+v"(d[i]) : "v"(1.0001), "v"(1e-9));
-            if (KIND == 5) asm volatile("v_mul_f32 %0, %0, %1" : "+v"(a[i].x) : "v"(m.x));
+            if (KIND == 0) asm volatile("v_fma_f32 %0, %0, %1, %2" : "+v"(a[i]) : "v"(m), "v"(c));
+            if (KIND == 1) asm volatile("v_mul_f32 %0, %0, %1" : "+v"(a[i]) : "v"(m));
+            if (KIND == 2) asm volatile("v_fma_f64 %0, %0, %1, %2" : "+v"(d[i]) : "v"(1.0001), "v"(1e-9));
         }
     }
     const long long t1 = clock64();
     float s = 0;
-    for (int i = 0; i < 8; i++) s += a[i].x + a[i].y + static_cast<float>(d[i]);
+    for (int i = 0; i < 8; i++) s += a[i] + static_cast<float>(d[i]);
     if ((threadIdx.x & 63) == 0) { out[2 * (threadIdx.x >> 6)] = t0; out[2 * (threadIdx.x >> 6) + 1] = t1; } // per wave: start, end
     if (s == 12345.678f) out[0] = 0;
 }
@@ -54,10 +49,7 @@ int main() {
     long long *d;
     hipMalloc(&d, 32 * sizeof(long long));
     run<0>("v_fma_f32", d);
-    run<5>("v_mul_f32", d);
-    run<1>("v_pk_fma_f32", d);
-    run<2>("v_pk_mul_f32", d);
-    run<3>("v_pk_add_f32", d);
-    run<4>("v_fma_f64", d);
+    run<1>("v_mul_f32", d);
+    run<2>("v_fma_f64", d);
     return 0;
 }

@@ -2,7 +2,10 @@
 assembly, builtins, assembly files) and wherever it lies -- a stand-alone probe that nothing builds counts like the library.
 
 Data is written through vector stores only.  The scalar data cache is not coherent with them, so a write through it (a scalar
-store, a scalar atomic, a write-back or discard of that cache) can lose or overtake the vector stores beside it."""
+store, a scalar atomic, a write-back or discard of that cache) can lose or overtake the vector stores beside it.
+
+Single-precision arithmetic is written one value per lane: some forms of the packed instructions (two f32 per instruction) have
+given wrong results on MI355X now and then, without an error."""
 import os
 import re
 
@@ -12,6 +15,7 @@ REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 SOURCE = re.compile(r"\.(hip|cu|cpp|cc|c|hpp|h|cuh|s|S|ll|py|sh|txt|cmake|mk)$|^Makefile$")
 FOLDERS = ("timemachine_amd", "include", "oracle", "scripts", "tests", "bench.py", "__graft_entry__.py")
 SCALAR_CACHE_WRITE = re.compile(r"(?:\b|_)s_(?:(?:scratch_|buffer_)?(?:store|atomic)_|dcache_(?:wb|discard))", re.IGNORECASE)
+PACKED_F32 = re.compile(r"\bv_pk_(?:add|mul|fma)_f32\b", re.IGNORECASE)
 
 
 def device_sources():
@@ -43,4 +47,16 @@ def test_the_scalar_cache_pattern_leaves_loads_and_vector_stores(op):
 
 def test_no_source_writes_through_the_scalar_data_cache():
     found = [h for path in device_sources() for h in hits(SCALAR_CACHE_WRITE, path)]
+    assert not found, "\n".join(found)
+
+
+@pytest.mark.parametrize("op", ["add", "mul", "fma"])
+def test_the_packed_f32_pattern_finds_every_kind(op):
+    assert PACKED_F32.search(f'asm volatile("v_pk_{op}_f32 %0, %0, %1" : "+v"(a))')
+    assert not PACKED_F32.search(f'asm volatile("v_pk_{op}_f16 %0, %0, %1" : "+v"(a))')
+    assert not PACKED_F32.search(f'asm volatile("v_{op}_f32 %0, %0, %1" : "+v"(a))')
+
+
+def test_no_source_holds_packed_f32_arithmetic():
+    found = [h for path in device_sources() for h in hits(PACKED_F32, path)]
     assert not found, "\n".join(found)
