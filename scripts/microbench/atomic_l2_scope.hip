@@ -1,6 +1,6 @@
 // Where does a global atomic of WORKGROUP scope execute on gfx950 -- in the issuing XCD's L2 (then adds from different XCDs to
 // one address lose updates: eight non-coherent L2s) or at the memory side like agent scope (then the sum is exact)?  And what
-// does each cost per wave instruction?    hipcc --offload-arch=gfx950 -O3 atomic_l2_scope.hip -o atomic_l2_scope
+// does each cost per wave instruction?    hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops atomic_l2_scope.hip -o atomic_l2_scope
 #include <hip/hip_runtime.h>
 #include <cstdio>
 template <int SCOPE> __global__ void k(unsigned long long *p, int reps, long long *cycles) {

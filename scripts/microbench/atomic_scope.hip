@@ -2,7 +2,7 @@
 // coherent with each other) vs workgroup scope (executed in the issuing XCD's L2).  The pattern imitates the tile kernel's
 // flush: 3072 waves, each issuing rounds of 64-lane atomics to 3 consecutive u64 per "atom", atoms spread over a
 // 23.5k-atom accumulator (one accumulator per XCD in the local variant).
-//   hipcc --offload-arch=gfx950 -O3 atomic_scope.hip -o atomic_scope && ./atomic_scope
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops atomic_scope.hip -o atomic_scope && ./atomic_scope
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>

@@ -1,5 +1,5 @@
 // wave_rol:1 / wave_ror:1 DPP controls on gfx950: which lane does lane l read?  (the rotation tile kernel passes the
-// row-force accumulators from lane to lane with them)   hipcc --offload-arch=gfx950 -O3 dpp_rotate.hip -o dpp_rotate
+// row-force accumulators from lane to lane with them)   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops dpp_rotate.hip -o dpp_rotate
 #include <hip/hip_runtime.h>
 #include <cstdio>
 __global__ void k(unsigned int *out) {

@@ -1,5 +1,5 @@
 // row_ror:n DPP control on gfx950: which lane does lane l read?  (the tile kernel's filter meets its rows through it)
-//   hipcc --offload-arch=gfx950 -O3 dpp_row_ror.hip -o dpp_row_ror
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops dpp_row_ror.hip -o dpp_row_ror
 #include <hip/hip_runtime.h>
 #include <cstdio>
 template <int N> __device__ __forceinline__ float ror(float v) {

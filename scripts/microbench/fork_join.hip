@@ -2,7 +2,7 @@
 // The MD step is  update(t-1) -> [list launch that only reads a flag: ~4 us] -> tiles(t): 55 us -> update(t).  Forked form:
 //   stream A: update -> (event E1) -> small -> (wait E2) -> update ...        stream B: (wait E1) -> long -> (event E2)
 // i.e. the small kernel and the long one both start behind the update; the next update waits for both.  What two cross-stream
-// dependencies per step cost decides whether this can pay.   hipcc --offload-arch=gfx950 -O3 scripts/microbench/fork_join.hip -o ... 
+// dependencies per step cost decides whether this can pay.   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops scripts/microbench/fork_join.hip -o ... 
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #define CHECK(x) do { hipError_t e_ = (x); if (e_ != hipSuccess) { printf("HIP error %s at %d\n", hipGetErrorString(e_), __LINE__); return 1; } } while (0)

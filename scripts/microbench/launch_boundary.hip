@@ -3,7 +3,7 @@
 // 256 x 1024-thread launch that does ~50 us of dependent FMAs, a 369 x 64-thread launch that touches 23.5k atoms), enqueued
 // (a) as plain stream launches and (b) as a graph of STEPS steps captured once and replayed.  Prints us per step for both, and
 // the same with the middle kernel removed (pure boundary cost).
-//   hipcc --offload-arch=gfx950 -O3 -o /tmp/launch_boundary scripts/microbench/launch_boundary.hip && /tmp/launch_boundary
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o /tmp/launch_boundary scripts/microbench/launch_boundary.hip && /tmp/launch_boundary
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>

@@ -1,5 +1,5 @@
 // Microbenchmark: LDS atomic throughput on gfx950 (cycles per wave-level instruction, all CUs busy, 16 waves/CU).
-// hipcc --offload-arch=gfx950 -O3 scripts/microbench/lds_atomics.hip -o gpurun_out/lds_atomics && gpurun_out/lds_atomics
+// hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops scripts/microbench/lds_atomics.hip -o gpurun_out/lds_atomics && gpurun_out/lds_atomics
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>

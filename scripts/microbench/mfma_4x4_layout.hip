@@ -1,5 +1,5 @@
 // v_mfma_f32_4x4x1_16b_f32 on gfx950: sixteen independent 4 x 4 outer products per instruction.  Which lane supplies what,
-// and where do the results land?   hipcc --offload-arch=gfx950 -O3 mfma_4x4_layout.hip -o mfma_4x4_layout
+// and where do the results land?   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops mfma_4x4_layout.hip -o mfma_4x4_layout
 //   claim checked:  lane l = 4 b + i supplies A[b][i] and B[b][i];  accumulator v of lane l = 4 b + j is D[b][v][j] = A[b][v] * B[b][j]
 #include <hip/hip_runtime.h>
 #include <cstdio>

@@ -1,5 +1,5 @@
 // v_mfma_f32_16x16x4_f32 on gfx950: operand and result layout, and the arithmetic error of a distance matrix computed as
-// |r|^2 - 2 r.c in f32 (the tile kernel's MFMA filter).   hipcc --offload-arch=gfx950 -O3 mfma_layout.hip -o mfma_layout
+// |r|^2 - 2 r.c in f32 (the tile kernel's MFMA filter).   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops mfma_layout.hip -o mfma_layout
 //   claim checked here:  A: lane l supplies A[row = l % 16][k = l / 16];  B: lane l supplies B[k = l / 16][col = l % 16];
 //                        D: accumulator v of lane l is D[row = 4 * (l / 16) + v][col = l % 16]
 #include <hip/hip_runtime.h>

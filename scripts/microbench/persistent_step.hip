@@ -1,7 +1,7 @@
 // Microbenchmark: what a PERSISTENT multi-step MD kernel would pay per step for its two device-wide barriers and for handing data
 // from one phase's writers to the next phase's readers across the eight (mutually non-coherent) XCD L2s of an MI355X -- the cost
 // floor of "several steps of a small system in ONE launch", measured before building it.
-//   hipcc --offload-arch=gfx950 -O3 scripts/microbench/persistent_step.hip -o gpurun_out/persistent_step && gpurun_out/persistent_step
+//   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops scripts/microbench/persistent_step.hip -o gpurun_out/persistent_step && gpurun_out/persistent_step
 // Per step: phase A every thread publishes one double, barrier, phase B every thread reads a double published by ANOTHER workgroup
 // (and checks it), barrier.  Variants: how the data moves (agent-scope atomic load / store, i.e. past the L2s; or plain accesses
 // bracketed by agent-scope release / acquire fences = L2 write-back + invalidate) and how many workgroups take part.

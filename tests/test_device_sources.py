@@ -5,9 +5,12 @@ Data is written through vector stores only.  The scalar data cache is not cohere
 store, a scalar atomic, a write-back or discard of that cache) can lose or overtake the vector stores beside it.
 
 Single-precision arithmetic is written one value per lane: some forms of the packed instructions (two f32 per instruction) have
-given wrong results on MI355X now and then, without an error."""
+given wrong results on MI355X now and then, without an error.  The compiler makes them from ordinary float code too, so the
+built libraries' device code is looked at as well."""
 import os
 import re
+import shutil
+import subprocess
 
 import pytest
 
@@ -60,3 +63,26 @@ def test_the_packed_f32_pattern_finds_every_kind(op):
 def test_no_source_holds_packed_f32_arithmetic():
     found = [h for path in device_sources() for h in hits(PACKED_F32, path)]
     assert not found, "\n".join(found)
+
+
+@pytest.mark.parametrize("lib", ["libtimemachine_amd.so", "libtimemachine_amd_rowblock.so"])
+def test_the_built_device_code_holds_no_packed_f32_arithmetic(lib, tmp_path):
+    objdump = os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "llvm", "bin", "llvm-objdump")
+    src = os.path.join(REPO, "timemachine_amd", "csrc", lib)
+    if not os.path.exists(objdump):
+        pytest.skip("no llvm-objdump")
+    if not os.path.exists(src):
+        import __graft_entry__
+
+        __graft_entry__.build()
+    copy = shutil.copy(src, tmp_path)
+    subprocess.run([objdump, "--offloading", copy], check=True, stdout=subprocess.DEVNULL)  # writes the code objects beside the copy
+    objects = sorted(p for p in tmp_path.iterdir() if "amdgcn" in p.name)
+    assert len(objects) >= 5
+    total = 0
+    for obj in objects:
+        text = subprocess.run([objdump, "-d", str(obj)], check=True, capture_output=True, text=True).stdout
+        total += text.count("v_fma_f32") + text.count("v_mul_f32")
+        packed = PACKED_F32.findall(text)
+        assert not packed, f"{obj.name}: {len(packed)} packed f32 instructions"
+    assert total > 1000  # the listing is one of the f32 kernels too
