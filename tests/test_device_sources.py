@@ -86,3 +86,51 @@ def test_the_built_device_code_holds_no_packed_f32_arithmetic(lib, tmp_path):
         packed = PACKED_F32.findall(text)
         assert not packed, f"{obj.name}: {len(packed)} packed f32 instructions"
     assert total > 1000  # the listing is one of the f32 kernels too
+
+
+LOAD = re.compile(r"\b(?:ds_read|ds_load|global_load|flat_load|buffer_load|scratch_load|s_load|s_buffer_load)\w*")
+COMMENT = re.compile(r"//[^\n]*|/\*.*?\*/", re.DOTALL)
+
+
+def asm_statements(text):
+    """the argument lists of the inline asm statements, comments taken out"""
+    text = COMMENT.sub("", text)
+    for m in re.finditer(r"\b(?:asm|__asm__)\b\s*(?:volatile|__volatile__)?\s*\(", text):
+        depth, i = 1, m.end()
+        while depth:
+            depth += {"(": 1, ")": -1}.get(text[i], 0)
+            i += 1
+        yield text[m.end():i - 1]
+
+
+def loads_without_their_wait(text):
+    # a statement may name its instructions through macros, and those through others
+    macros = dict(re.findall(r"#define (\w+)(?:\([^)]*\))?((?:[^\n]*\\\n)*[^\n]*)", COMMENT.sub("", text)))
+    loading = {m for m, body in macros.items() if LOAD.search(body)}
+    while True:
+        more = {m for m, body in macros.items() if any(re.search(rf"\b{k}\b", body) for k in loading)} | loading
+        if more == loading:
+            break
+        loading = more
+    return [s for s in asm_statements(text) if (LOAD.search(s) or any(re.search(rf"\b{k}\b", s) for k in loading)) and "s_waitcnt" not in s]
+
+
+def test_the_search_for_loads_without_their_wait():
+    read = 'ds_read_b64 %0, %1 offset:8'
+    assert loads_without_their_wait(f'asm volatile("{read}" : "=v"(v) : "v"(a)); asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(v));')
+    assert not loads_without_their_wait(f'asm volatile("{read}\\n\\ts_waitcnt lgkmcnt(0)" : "=&v"(v) : "v"(a));')
+    assert not loads_without_their_wait(f'// asm volatile("{read}")\nasm volatile("v_mov_b32 %0, %1" : "=v"(v) : "v"(a)); // {read}')
+    macro = f'#define READ(C) "{read}\\n\\t"\n#define READ_ALL READ(0) \\\n    READ(1)\n'
+    assert loads_without_their_wait(macro + 'asm volatile(READ_ALL : "=v"(v) : "v"(a));')
+    assert not loads_without_their_wait(macro + 'asm volatile(READ_ALL "s_waitcnt lgkmcnt(0)" : "=&v"(v) : "v"(a));')
+
+
+def test_every_load_in_inline_asm_is_waited_for_in_its_own_statement():
+    """The compiler takes an asm output as written when the statement ends: a load still under way behind it lands in a register
+    that may have been copied or given away meanwhile."""
+    found = []
+    for path in device_sources():
+        if path.endswith((".hip", ".hpp", ".h", ".cpp")):
+            with open(path, errors="replace") as fh:
+                found += [f"{os.path.relpath(path, REPO)}: {s}" for s in loads_without_their_wait(fh.read())]
+    assert not found, "\n".join(found)

@@ -94,47 +94,32 @@ template <typename Real, bool U, bool X, bool PP, bool DUAL> constexpr bool tile
 template <typename T> __device__ __forceinline__ unsigned int lds_offset(const T *p) {
     return static_cast<unsigned int>(reinterpret_cast<unsigned long>((__attribute__((address_space(3))) const void *)p));
 }
-// one ds_read_b64, issued and NOT waited for: the value is valid only after lds_wait14() on it
-template <int OFFSET> __device__ __forceinline__ double lds_read_f64_async(const unsigned int byte_offset) {
-    double v;
-    asm volatile("ds_read_b64 %0, %1 offset:%2" : "=v"(v) : "v"(byte_offset), "n"(OFFSET));
-    return v;
-}
-// (COL_BASE: byte distance of the column array from the row array, both addressed from the row array's base; SKIP_W: component
-// 3 is neither read nor waited for)
-template <int C, int ROW_STRIDE, int COL_STRIDE, int COL_BASE, bool SKIP_W = false> __device__ __forceinline__ void lds_read14(const unsigned int ra, const unsigned int ca, double (&ri)[7], double (&cj)[7]) {
-    if constexpr (C < 7) {
-        if constexpr (!(SKIP_W && C == 3)) {
-            ri[C] = lds_read_f64_async<C * ROW_STRIDE>(ra);
-            cj[C] = lds_read_f64_async<COL_BASE + C * COL_STRIDE>(ca);
-        }
-        lds_read14<C + 1, ROW_STRIDE, COL_STRIDE, COL_BASE, SKIP_W>(ra, ca, ri, cj);
-    }
-}
-template <int C, int ROW_STRIDE, int COL_STRIDE, int COL_BASE, bool SKIP_W = false> __device__ __forceinline__ void lds_read14(const unsigned int, const unsigned int, float (&)[7], float (&)[7]) {}
-// waits for every outstanding LDS operation of the wave; the values pass through the statement so that no use of them can
-// be scheduled in front of it
-template <bool SKIP_W = false> __device__ __forceinline__ void lds_wait14(double (&a)[7], double (&b)[7]) {
+// The operands of one pair: fourteen (SKIP_W: twelve, component 3 stays unread) single ds_read_b64 and the wait for them, in ONE
+// statement: the compiler takes an asm output as written when its statement ends, so a read that is still under way behind its
+// statement could land in a register that has been copied or given away meanwhile.  (Outputs are early-clobber: the addresses are
+// needed by the later reads.  COL_BASE: byte distance of the column array from the row array.)
+template <int ROW_STRIDE, int COL_STRIDE, int COL_BASE, bool SKIP_W = false> __device__ __forceinline__ void lds_read14(const unsigned int ra, const unsigned int ca, double (&ri)[7], double (&cj)[7]) {
+#define TM_READ_ROW(C) "ds_read_b64 %[r" #C "], %[ra] offset:%[ro" #C "]\n\t"
+#define TM_READ_COL(C) "ds_read_b64 %[c" #C "], %[ca] offset:%[co" #C "]\n\t"
+#define TM_READ_PAIR(C) TM_READ_ROW(C) TM_READ_COL(C)
+#define TM_READ_OUT(C) [r##C] "=&v"(ri[C]), [c##C] "=&v"(cj[C])
+#define TM_READ_OFF(C) [ro##C] "n"(C * ROW_STRIDE), [co##C] "n"(COL_BASE + C * COL_STRIDE)
     if constexpr (SKIP_W) {
-        asm volatile("s_waitcnt lgkmcnt(0)"
-                     : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[4]), "+v"(a[5]), "+v"(a[6]), "+v"(b[0]), "+v"(b[1]), "+v"(b[2]), "+v"(b[4]), "+v"(b[5]), "+v"(b[6]));
+        asm volatile(TM_READ_PAIR(0) TM_READ_PAIR(1) TM_READ_PAIR(2) TM_READ_PAIR(4) TM_READ_PAIR(5) TM_READ_PAIR(6) "s_waitcnt lgkmcnt(0)"
+                     : TM_READ_OUT(0), TM_READ_OUT(1), TM_READ_OUT(2), TM_READ_OUT(4), TM_READ_OUT(5), TM_READ_OUT(6)
+                     : [ra] "v"(ra), [ca] "v"(ca), TM_READ_OFF(0), TM_READ_OFF(1), TM_READ_OFF(2), TM_READ_OFF(4), TM_READ_OFF(5), TM_READ_OFF(6));
     } else {
-        asm volatile("s_waitcnt lgkmcnt(0)"
-                     : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3]), "+v"(a[4]), "+v"(a[5]), "+v"(a[6]), "+v"(b[0]), "+v"(b[1]), "+v"(b[2]),
-                       "+v"(b[3]), "+v"(b[4]), "+v"(b[5]), "+v"(b[6]));
+        asm volatile(TM_READ_PAIR(0) TM_READ_PAIR(1) TM_READ_PAIR(2) TM_READ_PAIR(3) TM_READ_PAIR(4) TM_READ_PAIR(5) TM_READ_PAIR(6) "s_waitcnt lgkmcnt(0)"
+                     : TM_READ_OUT(0), TM_READ_OUT(1), TM_READ_OUT(2), TM_READ_OUT(3), TM_READ_OUT(4), TM_READ_OUT(5), TM_READ_OUT(6)
+                     : [ra] "v"(ra), [ca] "v"(ca), TM_READ_OFF(0), TM_READ_OFF(1), TM_READ_OFF(2), TM_READ_OFF(3), TM_READ_OFF(4), TM_READ_OFF(5), TM_READ_OFF(6));
     }
+#undef TM_READ_OUT
+#undef TM_READ_OFF
+#undef TM_READ_PAIR
+#undef TM_READ_COL
+#undef TM_READ_ROW
 }
-template <bool SKIP_W = false> __device__ __forceinline__ void lds_wait14(float (&)[7], float (&)[7]) {}
-// experiment (TM_SPLIT_WAIT, flat items): the six coordinate reads are issued first and waited for alone -- LDS returns in order --, so
-// the displacement and d^2 issue while charge, sigma and epsilon are still on their way
-__device__ __forceinline__ void lds_wait_first6_of12(double (&a)[7], double (&b)[7]) {
-    asm volatile("s_waitcnt lgkmcnt(6)" : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(b[0]), "+v"(b[1]), "+v"(b[2]));
-}
-__device__ __forceinline__ void lds_wait_first6_of12(float (&)[7], float (&)[7]) {}
-__device__ __forceinline__ void lds_wait_rest6(float (&)[7], float (&)[7]) {}
-__device__ __forceinline__ void lds_wait_rest6(double (&a)[7], double (&b)[7]) {
-    asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(a[4]), "+v"(a[5]), "+v"(a[6]), "+v"(b[4]), "+v"(b[5]), "+v"(b[6]));
-}
+template <int ROW_STRIDE, int COL_STRIDE, int COL_BASE, bool SKIP_W = false> __device__ __forceinline__ void lds_read14(const unsigned int, const unsigned int, float (&)[7], float (&)[7]) {}
 // branch-probability hint for the block placement of the f64 kernels (measured: +0.5 % there, -2 % on the f32 kernels)
 template <bool ON> __device__ __forceinline__ bool hint(const bool c, const bool expected) {
     if constexpr (ON) {
@@ -1354,16 +1339,7 @@ __global__ __launch_bounds__((64 * TileShape<Real, tile_wide<Real, COMPUTE_U, CO
 #else
                     const unsigned int ra = lds_offset(&s_row[0][0]) + pi * 8u, ca = lds_offset(&s_row[0][0]) + pj * 8u;
 #endif
-                    lds_read14<0, TILE * 8, NB_CHUNK * 8, static_cast<int>(offsetof(WaveLds, col) - offsetof(WaveLds, row)), FLAT>(ra, ca, ri, cj);
-#ifdef TM_SPLIT_WAIT
-                    if constexpr (FLAT) {
-                        lds_wait_first6_of12(ri, cj);
-                    } else {
-                        lds_wait14<FLAT>(ri, cj);
-                    }
-#else
-                    lds_wait14<FLAT>(ri, cj);
-#endif
+                    lds_read14<TILE * 8, NB_CHUNK * 8, static_cast<int>(offsetof(WaveLds, col) - offsetof(WaveLds, row)), FLAT>(ra, ca, ri, cj);
                 } else {
 #pragma unroll
                     for (int c = 0; c < 7; c++) {
@@ -1397,11 +1373,6 @@ __global__ __launch_bounds__((64 * TileShape<Real, tile_wide<Real, COMPUTE_U, CO
                         energy2 += float_to_fixed_energy_hot<Real>(o2.u);
                     }
                 }
-#ifdef TM_SPLIT_WAIT
-                if constexpr (sizeof(Real) == 8 && TM_LDS_SINGLE_READS && FLAT) {
-                    lds_wait_rest6(ri, cj);
-                }
-#endif
 #ifdef TM_TIMING_BATCH
                 asm volatile("" : "+v"(ddx), "+v"(ddy), "+v"(ddz)); // (the stamp must not be hoisted over the arithmetic)
                 {

@@ -133,22 +133,24 @@ struct RbEsTable { // the workgroup's LDS copy of the force-factor table (nb_es_
     }
 };
 
-// row operands of one pair: single ds_read_b64 issued from asm (the compiler would pair them into ds_read2_b64, which the LDS
-// serves at half rate), component stride 32 rows * 8 bytes
-template <int C, bool SKIP_W> __device__ __forceinline__ void rb_read_row(const unsigned int addr, double (&ri)[7]) {
-    if constexpr (C < 7) {
-        if constexpr (!(SKIP_W && C == 3)) {
-            ri[C] = lds_read_f64_async<C * TILE * 8>(addr);
-        }
-        rb_read_row<C + 1, SKIP_W>(addr, ri);
-    }
-}
-template <bool SKIP_W> __device__ __forceinline__ void rb_wait_row(double (&a)[7]) {
+// row operands of one pair: single ds_read_b64 (the compiler would pair them into ds_read2_b64, which the LDS serves at half rate)
+// and the wait for them in one statement, as in lds_read14; component stride 32 rows * 8 bytes
+template <bool SKIP_W> __device__ __forceinline__ void rb_read_row(const unsigned int addr, double (&ri)[7]) {
+#define TM_READ_ROW(C) "ds_read_b64 %[r" #C "], %[a] offset:%[o" #C "]\n\t"
+#define TM_READ_OUT(C) [r##C] "=&v"(ri[C])
+#define TM_READ_OFF(C) [o##C] "n"(C * TILE * 8)
     if constexpr (SKIP_W) {
-        asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[4]), "+v"(a[5]), "+v"(a[6]));
+        asm volatile(TM_READ_ROW(0) TM_READ_ROW(1) TM_READ_ROW(2) TM_READ_ROW(4) TM_READ_ROW(5) TM_READ_ROW(6) "s_waitcnt lgkmcnt(0)"
+                     : TM_READ_OUT(0), TM_READ_OUT(1), TM_READ_OUT(2), TM_READ_OUT(4), TM_READ_OUT(5), TM_READ_OUT(6)
+                     : [a] "v"(addr), TM_READ_OFF(0), TM_READ_OFF(1), TM_READ_OFF(2), TM_READ_OFF(4), TM_READ_OFF(5), TM_READ_OFF(6));
     } else {
-        asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(a[0]), "+v"(a[1]), "+v"(a[2]), "+v"(a[3]), "+v"(a[4]), "+v"(a[5]), "+v"(a[6]));
+        asm volatile(TM_READ_ROW(0) TM_READ_ROW(1) TM_READ_ROW(2) TM_READ_ROW(3) TM_READ_ROW(4) TM_READ_ROW(5) TM_READ_ROW(6) "s_waitcnt lgkmcnt(0)"
+                     : TM_READ_OUT(0), TM_READ_OUT(1), TM_READ_OUT(2), TM_READ_OUT(3), TM_READ_OUT(4), TM_READ_OUT(5), TM_READ_OUT(6)
+                     : [a] "v"(addr), TM_READ_OFF(0), TM_READ_OFF(1), TM_READ_OFF(2), TM_READ_OFF(3), TM_READ_OFF(4), TM_READ_OFF(5), TM_READ_OFF(6));
     }
+#undef TM_READ_ROW
+#undef TM_READ_OUT
+#undef TM_READ_OFF
 }
 
 template <typename Real, bool INSIDE_SWITCH>
@@ -597,8 +599,7 @@ __global__ __launch_bounds__(RB_THREADS, (RB_WAVES * RB_WGS_PER_CU) / 4) void k_
                     Real ri[7];
                     if constexpr (F64) {
                         const unsigned int a = lds_offset(&rows.row[0][0]) + pi * 8u;
-                        rb_read_row<0, FLAT>(a, ri);
-                        rb_wait_row<FLAT>(ri);
+                        rb_read_row<FLAT>(a, ri);
                     } else {
 #pragma unroll
                         for (int c = 0; c < 7; c++) {
