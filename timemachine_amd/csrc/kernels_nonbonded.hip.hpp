@@ -34,8 +34,8 @@ namespace tmamd {
 // Waves per SIMD the tile kernel is register-budgeted for (512 / waves VGPRs per lane).  f64: 4 waves = 128 registers since the
 // general filter paths became asm statements too (round 3: in plain C++ they took the whole kernel from 130 to 156 registers
 // and 4 waves meant 60 spilled dwords; measured then: 63.2 / 68 us against 63.9 / 62 at 3 waves; now 55.9 against 58.9 on a bare
-// tile launch, 57.2 against 57.8 with a step's bonded terms on board).  f32: ~100 registers -> 4 waves (5 would fit with 96,
-// but only in a workgroup shape whose item pools are too small, see TileShape).
+// tile launch, 57.2 against 57.8 with a step's bonded terms on board).  f32: 72 to 114 registers -> 4 waves (the
+// forces-only kernel's 92 would fit 5, but only in a workgroup shape whose item pools are too small, see TileShape).
 template <typename Real> struct TileWaves {
 #ifndef TM_TILE_WAVES_F64
 #define TM_TILE_WAVES_F64 4
